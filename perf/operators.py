@@ -40,9 +40,9 @@ def listed():
         # a full-resolution layer at batch 2: the largest of a training step
         dict(name='backward/full', op='backward', N=2, C=32, D=128, H=128, W=128, fmt='int8', g1=True, g2=False, K=0),
         # a small product of odd sizes for every item of a batch
-        dict(name='product/odd', op='product', B=3, M=61, N=136, K=1000, dtype='f32', total=False),
+        dict(name='product/odd', op='product', B=3, M=61, N=136, K=1000, dtype='bf16', total=False),
         # a large one, bound by the matrix cores
-        dict(name='product/8192', op='product', B=1, M=8192, N=8192, K=8192, dtype='bf16', total=False),
+        dict(name='product/8192', op='product', B=1, M=8192, N=8192, K=8192, dtype='f32', total=False),
         # weight gradient of the transposed convolution of a thick-slice stage (1, 2, 2): small and odd
         dict(name='tu_wgrad/odd', op='tu_wgrad', N=1, Cin=40, Cout=24, D=5, H=7, W=9, kt=1),
         # that of the last decoder stage (64^3 -> 128^3) at batch 2
