@@ -285,7 +285,7 @@ extern "C" int wmh_act8_unpack(const uint8_t* codes, const uint8_t* scales, int 
 //   apply   dy = gamma rstd (dz - sum dz / S - xh sum(dz xh) / S), and sum dy
 // Both passes are bound by the memory: a lane takes four voxels a step (one dword of codes, 16 bytes of every other source) and U steps with their
 // loads issued together; the sources are template parameters so that no branch stands between the loads.  Four terms are added in 32 bits, the
-// rest in 64, in a fixed order.  KT: classes of the head a kernel is built for (0, 2, 4); an odd one out reads class 0 again with weight 0.
+// rest in 64, in a fixed order.  KT: classes of the head a kernel is built for (a padded class with weight 0 would make NaN of an infinite gradient).
 #define ACT8_MAXK 4
 struct Act8Bwd {
     const uint8_t* codes; const uint8_t* scales; const float* ss; const float* mr; const float* gamma;
@@ -315,8 +315,8 @@ struct Act8Row {
         g1 = (SRC & 1) ? a.g1 + nc * a.S : nullptr; g2 = (SRC & 2) ? a.g2 + nc * a.S : nullptr;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
-            dl[k] = a.dl + (n * a.K + (k < a.K ? k : 0)) * a.S;
-            w[k] = k < a.K ? a.wseg[k * a.C + c] : 0.f;
+            dl[k] = a.dl + (n * KT + k) * a.S;
+            w[k] = a.wseg[k * a.C + c];
         }
         sc = a.ss[2 * nc]; sh = a.ss[2 * nc + 1]; mean = a.mr[2 * nc]; rstd = a.mr[2 * nc + 1]; slope = a.slope;
     }
@@ -533,8 +533,7 @@ __global__ __launch_bounds__(512) void act8_bwd_row_kernel(const Act8Bwd a) {
     if (a.dbias) a.dbias[c] = (float)acc;
     if (a.dwseg)
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
-            if (j < a.K) a.dwseg[j * a.C + c] = (float)sk[j];
+        for (int j = 0; j < KT; ++j) a.dwseg[j * a.C + c] = (float)sk[j];
 }
 // Parameter gradients: one wave per channel over the n rows and their slices.
 __global__ __launch_bounds__(64) void act8_bwd_param_kernel(const Act8Bwd a) {
@@ -586,20 +585,23 @@ static void launch_bwd(const Act8Bwd& a, unsigned rows, hipStream_t st) {
     hipLaunchKernelGGL((act8_bwd_apply_kernel<FMT, SRC, KT>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL(act8_bwd_param_kernel, dim3(a.C), dim3(64), 0, st, a);
 }
+template <int FMT, int KT>
+static void launch_bwd_sources(const Act8Bwd& a, unsigned rows, hipStream_t st) {
+    switch ((a.g1 ? 1 : 0) + (a.g2 ? 2 : 0)) {
+        case 0: if constexpr (KT > 0) launch_bwd<FMT, 0, KT>(a, rows, st); break;
+        case 1: launch_bwd<FMT, 1, KT>(a, rows, st); break;
+        case 2: launch_bwd<FMT, 2, KT>(a, rows, st); break;
+        default: launch_bwd<FMT, 3, KT>(a, rows, st); break;
+    }
+}
 template <int FMT>
 static void launch_bwd_form(const Act8Bwd& a, unsigned rows, hipStream_t st) {
-    switch (((a.K + 1) / 2) * 4 + (a.g1 ? 1 : 0) + (a.g2 ? 2 : 0)) {
-        case 1: launch_bwd<FMT, 1, 0>(a, rows, st); break;
-        case 2: launch_bwd<FMT, 2, 0>(a, rows, st); break;
-        case 3: launch_bwd<FMT, 3, 0>(a, rows, st); break;
-        case 4: launch_bwd<FMT, 0, 2>(a, rows, st); break;
-        case 5: launch_bwd<FMT, 1, 2>(a, rows, st); break;
-        case 6: launch_bwd<FMT, 2, 2>(a, rows, st); break;
-        case 7: launch_bwd<FMT, 3, 2>(a, rows, st); break;
-        case 8: launch_bwd<FMT, 0, 4>(a, rows, st); break;
-        case 9: launch_bwd<FMT, 1, 4>(a, rows, st); break;
-        case 10: launch_bwd<FMT, 2, 4>(a, rows, st); break;
-        default: launch_bwd<FMT, 3, 4>(a, rows, st); break;
+    switch (a.K) {
+        case 0: launch_bwd_sources<FMT, 0>(a, rows, st); break;
+        case 1: launch_bwd_sources<FMT, 1>(a, rows, st); break;
+        case 2: launch_bwd_sources<FMT, 2>(a, rows, st); break;
+        case 3: launch_bwd_sources<FMT, 3>(a, rows, st); break;
+        default: launch_bwd_sources<FMT, 4>(a, rows, st); break;
     }
 }
 extern "C" int wmh_act8_in_lrelu_bwd(const uint8_t* codes, const uint8_t* scales, int fmt, const float* ss, const float* mean_rstd, const float* gamma,
