@@ -12,7 +12,8 @@ nearest even.  A block that holds an infinity or a NaN reads NaN as a whole.
   convtranspose_weight_gradient        that product as the weight gradient of a transposed convolution (kernel = stride)
 
 Calls are asynchronous on torch's current stream of the tensors' device; outputs and workspaces come from torch's allocator unless given.
-There is no CPU path.  UNetTrainer(checkpoint8=..., tu_wgrad=...) is what uses them in training.
+There is no CPU path, and nothing is recorded for autograd: a tensor that requires grad is refused while grad mode is on.
+UNetTrainer(checkpoint8=..., tu_wgrad=...) is what uses them in training.
 """
 from collections import namedtuple
 
@@ -45,6 +46,7 @@ class Act8:
     """A packed tensor: `shape` of what it stands for ([N, C, ...]), `codes` [N, C, pitch] (torch.int8 or torch.float8_e4m3fn; zero behind a row's
     end) and exponent bytes `scales` [N, C, scale pitch] (uint8; 1 to 249, or 255 for a block that is not finite)."""
     __slots__ = ('codes', 'scales', 'shape', 'length')
+    requires_grad = False                                       # (to autograd; _device)
 
     def __init__(self, codes, scales, shape):
         shape = tuple(map(int, shape))
@@ -88,13 +90,19 @@ class Act8:
 
 
 def _device(what, first, *tensors):
-    """The HIP device all of these are on."""
-    dev = first.device
+    """The HIP device all of these are on.  With grad mode on none of them may require grad: its gradient would silently be missing."""
+    dev, grad = first.device, torch.is_grad_enabled()
+    lost = grad and first.requires_grad
+    for t in tensors:
+        if t is not None:
+            if t.device != dev:
+                raise ValueError('%s: tensors on %s and %s' % (what, dev, t.device))
+            if grad and t.requires_grad:
+                lost = True
+    if lost:
+        raise RuntimeError('%s records nothing for autograd, and one of its tensors requires grad: detach() it or call under torch.no_grad()' % what)
     if dev.type != 'cuda':
         raise RuntimeError('%s needs a HIP device; there is no CPU path' % what)
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError('%s: tensors on %s and %s' % (what, dev, t.device))
     return dev
 
 
