@@ -26,6 +26,14 @@ def _newer(a, b):
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
 
 
+def _read(path):
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def build_library(force=False, verbose=True, diag=True):
     """The product library and (diag=True) the diagnostic one; returns the product library's path."""
     lib = _build_one(LIB, 'obj', [], force, verbose)
@@ -43,9 +51,11 @@ def _build_one(LIB, objname, extra_flags, force, verbose):
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace('.hip', '.o'))
-        # (an object without its .res file -- the resource remarks -- is recompiled: the JSON below is rebuilt from those files)
-        if force or _newer(s, o) or any(_newer(d, o) for d in deps) or not os.path.exists(o[:-2] + '.res'):
-            jobs.append([HIPCC] + FLAGS + extra_flags + ['-c', s, '-o', o])
+        cmd = [HIPCC] + FLAGS + extra_flags + ['-c', s, '-o', o]
+        # (an object without its .res file -- the resource remarks -- is recompiled: the JSON below is rebuilt from those files; so is one that
+        # another command line made)
+        if force or _newer(s, o) or any(_newer(d, o) for d in deps) or not os.path.exists(o[:-2] + '.res') or _read(o[:-2] + '.cmd') != '\0'.join(cmd):
+            jobs.append(cmd)
             relink = True
         objs.append(o)
     # the translation units are independent: a few compilers side by side (WMH_BUILD_JOBS, default 4 -- each hipcc peaks at ~1.5 GB)
@@ -68,6 +78,8 @@ def _build_one(LIB, objname, extra_flags, force, verbose):
             raise subprocess.CalledProcessError(proc.returncode, cmd)
         with open(cmd[-1][:-2] + '.res', 'w') as f:         # <object>.res: the unit's resource remarks
             f.write('\n'.join(remarks) + '\n')
+        with open(cmd[-1][:-2] + '.cmd', 'w') as f:         # <object>.cmd: what made it
+            f.write('\0'.join(cmd))
     res = {}
     for o in objs:
         unit, cur = os.path.basename(o)[:-2], None
@@ -90,7 +102,7 @@ def _build_one(LIB, objname, extra_flags, force, verbose):
                     cur[key] = int(v.strip())
     with open(LIB[:-3] + '.resources.json', 'w') as f:
         json.dump(res, f, indent=0, sort_keys=True)
-    if relink:
+    if relink or any(_newer(o, LIB) for o in objs):
         cmd = [HIPCC, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs
         if verbose:
             print(' '.join(cmd), flush=True)
