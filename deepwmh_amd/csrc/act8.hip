@@ -9,7 +9,6 @@
 template <bool FAR, typename T> __device__ __forceinline__ T act8_ld(const T* p) { if constexpr (FAR) return __builtin_nontemporal_load(p); else return *p; }
 template <bool FAR, typename T> __device__ __forceinline__ void act8_st(const T& v, T* p) { if constexpr (FAR) __builtin_nontemporal_store(v, p); else *p = v; }
 static inline bool act8_far(size_t bytes) { return bytes > (size_t)192 << 20; }
-static inline unsigned cdivu(size_t a, size_t b) { return (unsigned)((a + b - 1) / b); }
 
 // ---- pack -------------------------------------------------------------------------------------------------------------------------------
 // 32 lanes x 4 values = one block, so that loads and stores are contiguous over a wave and the maximum stays inside half a wave.  A half-wave takes
@@ -57,7 +56,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const typename E::T* __r
             }
             const unsigned m0 = act8_abs_bits(z[u][0]), m1 = act8_abs_bits(z[u][1]), m2 = act8_abs_bits(z[u][2]), m3 = act8_abs_bits(z[u][3]);
             const unsigned m01 = m0 > m1 ? m0 : m1, m23 = m2 > m3 ? m2 : m3;
-            const unsigned byte = act8_byte<FMT>(act8_lanes_max<false>(m01 > m23 ? m01 : m23));
+            const unsigned byte = act8_byte<FMT>(act8_lanes_max(m01 > m23 ? m01 : m23));
             const float inv = act8_inverse(byte);
             unsigned w = act8_encode4<FMT>(z[u][0] * inv, z[u][1] * inv, z[u][2] * inv, z[u][3] * inv, byte == 255u);
             if (!WHOLE && FMT == WMH_ACT8_E4M3 && byte == 255u)                                     // the padding stays zero

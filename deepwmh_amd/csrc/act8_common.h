@@ -71,9 +71,8 @@ __device__ __forceinline__ unsigned act8_next(unsigned c, bool up) {
         return m ? c - 1 : (up ? 0x01u : 0x81u);
     }
 }
-// Largest of 32 (ALL: 64) lanes in all of them: four steps inside a row of 16, then rows against each other (gfx950's swap: even rows of one register
+// Largest of 32 lanes in all of them: four steps inside a row of 16, then rows against each other (gfx950's swap: even rows of one register
 // against odd rows of another); no LDS crossbar.
-template <bool ALL>
 __device__ __forceinline__ unsigned act8_lanes_max(unsigned m) {
 #define ACT8_DPP_MAX(CTRL) { const unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)m, CTRL, 0xF, 0xF, true); m = m > o ? m : o; }
     ACT8_DPP_MAX(0xB1)                // neighbours
@@ -82,12 +81,7 @@ __device__ __forceinline__ unsigned act8_lanes_max(unsigned m) {
     ACT8_DPP_MAX(0x140)               // row mirrored
 #undef ACT8_DPP_MAX
     const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-    m = a[0] > a[1] ? a[0] : a[1];
-    if constexpr (ALL) {
-        const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-        m = b[0] > b[1] ? b[0] : b[1];
-    }
-    return m;
+    return a[0] > a[1] ? a[0] : a[1];
 }
 // The same over the 32 even and the 32 odd lanes apart.
 __device__ __forceinline__ unsigned act8_parity_max(unsigned m) {

@@ -719,7 +719,7 @@ __global__ __launch_bounds__(512, 2) void act8_tu_wgrad_kernel(const Act8Tu a) {
             const unsigned m0_ = act8_abs_bits(v[0]), m1_ = act8_abs_bits(v[1]), m2_ = act8_abs_bits(v[2]), m3_ = act8_abs_bits(v[3]);
             const unsigned ma = m0_ > m1_ ? m0_ : m1_, mb = m2_ > m3_ ? m2_ : m3_;
             m = ma > mb ? ma : mb;
-            m = u < NX ? act8_lanes_max<false>(m) : act8_parity_max(m);
+            m = u < NX ? act8_lanes_max(m) : act8_parity_max(m);
             const unsigned byte = act8_byte<WMH_ACT8_E4M3>(m);
             const float inv = act8_inverse(byte);
             const unsigned code = act8_encode4<WMH_ACT8_E4M3>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, byte == 255u);
