@@ -1,4 +1,5 @@
-"""GPU tests of calls of the 8-bit checkpoint operators at the edges of what they accept."""
+"""GPU tests of calls of the 8-bit checkpoint operators at the edges of what they accept: sizes of a real training step, infinite gradients, scales at
+both ends of the range, batches of many small products."""
 import numpy as np
 import pytest
 import torch
@@ -7,7 +8,7 @@ import test_gpu_act8 as base
 from oracle import act8 as oa
 
 pytestmark = pytest.mark.gpu
-SLOPE = base.SLOPE
+U, HALF, SLOPE = base.U, base.HALF, base.SLOPE
 
 
 # ---- a head whose logit gradient is not finite ---------------------------------------------------------------------------------------------
@@ -39,3 +40,53 @@ def test_backward_of_an_infinite_logit_gradient(K, shape):
             assert np.array_equal(np.isfinite(g), ~off) and np.array_equal(g[off], w[off]), (name, k)
         dy = base._np(got.dy).reshape(N, C, S)
         assert not np.isfinite(dy[0]).any() and np.isfinite(dy[1:]).all()
+
+
+# ---- products ------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dims', [(1, 300, 520, 200), (3, 61, 136, 1000), (1, 512, 512, 1024), (1, 1030, 4100, 520), (1, 3590, 3601, 4480), (1, 64, 256, 40000)],
+                         ids=lambda d: 'x'.join(map(str, d)))
+def test_bfloat16_product_is_off_by_its_results_rounding(dims):
+    """Of random terms.  A result's rounding to bfloat16 is uniform over a step of at most 2^-7 of it: 2^-7 / sqrt(12) = 2.26e-3 in the norm at most.
+    In front of it eight products lose up to seven terms' bits below 2^-13 of the largest, toward zero, which for products of normal variables (the
+    largest of eight: 2.5) is 2.5 2^-13 sqrt(7 / 3) of the sum's own sqrt(8): 1.7e-4.  Together 2.27e-3."""
+    from deepwmh_amd import act8
+    B, M, N, K = dims
+    g = torch.Generator(device='cuda').manual_seed(31)
+    a, b = (act8.pack(torch.randn(B, r, K, device='cuda', generator=g), 'e4m3') for r in (M, N))
+    c = torch.matmul(act8.unpack(a).double(), act8.unpack(b).double().transpose(1, 2).contiguous())
+    for total in (False, True):
+        want = c.sum(0) if total else c
+        got = act8.product(a, b, dtype=torch.bfloat16, sum_batches=total).double()
+        assert float((got - want).norm() / want.norm()) <= 2.3e-3
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('dims', [(40, 35, 300), (20, 40, 300), (300, 70, 9000), (1100, 4200, 130), (3500, 3600, 260), (3500, 3600, 4200)],
+                         ids=lambda d: 'x'.join(map(str, d)))
+def test_products_of_scales_over_the_whole_range(dims, dtype):
+    """Rows of a and b with exponent bytes from the smallest to nearly the largest, so that a product of blocks lies anywhere between 2^-250 and 2^240."""
+    from deepwmh_amd import act8
+    M, N, K = dims
+    g = torch.Generator(device='cuda').manual_seed(32)
+    a, b = (torch.randn(1, r, K, device='cuda', generator=g, dtype=torch.float64) for r in (M, N))
+    for t in (a, b):
+        e = torch.randint(-124, 125, (1, t.shape[1], -(-K // 128)), device='cuda', generator=g).double()
+        e[:, ::2] = e[:, ::2, :1]                               # every second row of one size, the others with blocks of any
+        t *= torch.exp2(e).repeat_interleave(128, -1)[..., :K]
+    a, b = (act8.pack(t.float().clamp(-2.0 ** 127, 2.0 ** 127), 'e4m3') for t in (a, b))
+    assert int(a.scales[..., :-(-K // 128)].min()) <= 2 and int(a.scales.max()) >= 240
+    va, vb = act8.unpack(a).double(), act8.unpack(b).double()
+    c, mag = (torch.matmul(x, y.transpose(1, 2).contiguous())[0] for x, y in ((va, vb), (va.abs(), vb.abs())))
+    got = act8.product(a, b, dtype=dtype)[0].double()
+    # as for ordinary sizes; and a number below 2^-126, a product of two codes or a sum that is joined or stored, may be lost
+    tol = min(-(-K // 128) * 2 + 64, 600) * 2.0 ** -23 * mag + HALF[dtype] * c.abs() + (K + 300) * 2.0 ** -126
+    if dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -10 * mag
+    else:                                                       # codes widened with their scale are bfloat16 numbers: so may one of them below 2^-126
+        la, lb = (t.abs() * (t.abs() < 2.0 ** -126) for t in (va, vb))
+        tol = tol + torch.matmul(la, vb.abs().transpose(1, 2).contiguous())[0] + torch.matmul(va.abs(), lb.transpose(1, 2).contiguous())[0]
+    fits, over = mag < 2.0 ** 127, c.abs() >= 2.0 ** 129
+    assert int(fits.sum()) > M * N // 8 and not bool(torch.isfinite(got[over]).any())
+    assert bool(torch.isfinite(got[fits]).all()) and bool(((got - c).abs() <= tol)[fits].all())
+    small = fits & (c.abs() > 2.0 ** -100) & (mag < 2.0 ** 100) & (c.abs() > mag / 16)
+    assert int(small.sum()) > M * N // 64 and bool((got[small] != 0).all())
