@@ -90,3 +90,21 @@ def test_products_of_scales_over_the_whole_range(dims, dtype):
     assert bool(torch.isfinite(got[fits]).all()) and bool(((got - c).abs() <= tol)[fits].all())
     small = fits & (c.abs() > 2.0 ** -100) & (mag < 2.0 ** 100) & (c.abs() > mag / 16)
     assert int(small.sum()) > M * N // 64 and bool((got[small] != 0).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('dims', [(256, 64, 64, 512), (200, 40, 200, 700), (192, 33, 33, 130), (211, 61, 136, 1000), (6, 40, 8192, 260), (300, 33, 257, 129), (64, 128, 96, 2048)],
+                         ids=lambda d: 'x'.join(map(str, d)))
+def test_products_of_many_small_items(dims, dtype):
+    base.test_product_of_larger_odd_sizes(dims, dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_a_product_gives_the_same_bits_between_other_work(dtype):
+    from deepwmh_amd import act8
+    g = torch.Generator(device='cuda').manual_seed(33)
+    sets = [tuple(act8.pack(torch.randn(B, r, K, device='cuda', generator=g), 'e4m3') for r in (M, N)) for B, M, N, K in ((3, 61, 136, 1000), (1, 300, 500, 3000), (2, 17, 90, 9000))]
+    want = [act8.product(a, b, dtype=dtype) for a, b in sets]
+    for k in range(30):
+        for i in (0, 1, 2) if k % 2 else (2, 0, 1):
+            assert torch.equal(act8.product(*sets[i], dtype=dtype), want[i])
