@@ -108,3 +108,122 @@ def test_a_product_gives_the_same_bits_between_other_work(dtype):
     for k in range(30):
         for i in (0, 1, 2) if k % 2 else (2, 0, 1):
             assert torch.equal(act8.product(*sets[i], dtype=dtype), want[i])
+
+
+# ---- tensors of a real step ----------------------------------------------------------------------------------------------------------------
+LONG = 127 * 129 * 131                                          # an odd row of 2.1 million; 24 of them are past the 192 MB where accesses pass the caches
+
+
+def _quantise(z, fmt):
+    """float64 [R, L] finite -> code values [R, L], exponents [R, blocks] (written for the GPU, from the definition)."""
+    R, L = z.shape
+    nb = -(-L // 128)
+    z = torch.nn.functional.pad(z, (0, nb * 128 - L)).view(R, nb, 128)
+    top = 127.0 if fmt == 'int8' else 448.0
+    high = z.abs().amax(-1)
+    m, k = torch.frexp(high / top)
+    e = torch.where(high == 0, -126, torch.where(m == 0.5, k - 1, k).clamp(min=-126))
+    q = z / torch.exp2(e.double())[..., None]
+    if fmt == 'int8':
+        codes = q.round()
+    else:
+        step = torch.exp2((torch.frexp(q).exponent - 1).clamp(min=-6).double() - 3)
+        codes = (q / step).round() * step
+    return codes.view(R, -1)[:, :L], e
+
+
+def _values(codes, e):
+    return codes * torch.exp2(e.double()).repeat_interleave(128, -1)[:, :codes.shape[1]]
+
+
+def _grid(fmt):
+    if fmt == 'int8':
+        return torch.arange(-127, 128, device='cuda', dtype=torch.float64)
+    m = torch.arange(127, dtype=torch.float64)
+    mag = torch.where(m < 8, m * 2.0 ** -9, (8 + m % 8) * torch.exp2(torch.floor(m / 8) - 10))
+    return torch.cat([-mag.flip(0)[:-1], mag]).cuda()
+
+
+def _kept(z, codes, e, sc, sh, fmt):
+    """codes with those on the wrong side of z sc + sh = 0 moved to the neighbour on z's."""
+    grid = _grid(fmt)
+    v = _values(codes, e)
+    want, got = z * sc + sh > 0, v * sc + sh > 0
+    at = torch.searchsorted(grid, codes.contiguous())
+    moved = grid[(at + torch.where(want == (sc > 0), 1, -1)).clamp(0, grid.numel() - 1)]
+    return torch.where(want != got, moved, codes)
+
+
+def _long(C, g, dtype=torch.float32):
+    x = torch.randn(1, C, LONG, device='cuda', generator=g)
+    x *= torch.exp(torch.randn(1, C, 1, device='cuda', generator=g))
+    x += torch.randn(1, C, 1, device='cuda', generator=g)
+    ss = torch.stack([1 + 0.3 * torch.randn(1, C, device='cuda', generator=g), torch.randn(1, C, device='cuda', generator=g)], -1)
+    return x.to(dtype), ss
+
+
+@pytest.mark.parametrize('mode', ['plain', 'activate', 'keep_sign'])
+@pytest.mark.parametrize('fmt', ['int8', 'e4m3'])
+@pytest.mark.parametrize('dtype,C', [(torch.float32, 24), (torch.bfloat16, 48)])
+def test_pack_and_unpack_past_the_caches(dtype, C, fmt, mode):
+    from deepwmh_amd import act8
+    x, ss = _long(C, torch.Generator(device='cuda').manual_seed(34), dtype)
+    assert x.numel() * x.element_size() > 192 << 20
+    ck = act8.pack(x, fmt, ss=None if mode == 'plain' else ss, slope=SLOPE, keep_sign=mode == 'keep_sign')
+    nb = -(-LONG // 128)
+    backs = [act8.unpack(ck, dtype), act8.unpack(ck, dtype, ss=ss, slope=SLOPE)]
+    assert not bool(ck.codes[..., LONG:].float().any()) and not bool(ck.scales[..., nb:].any())
+    slope = torch.tensor(SLOPE, device='cuda')
+    for c in range(C):
+        z, sc, sh = x[0, c].double()[None], ss[0, c, 0].double(), ss[0, c, 1].double()
+        if mode == 'activate':
+            z = (z * sc + sh).float()                           # (a float64 product of two float32 is exact)
+            z = torch.where(z > 0, z, z * slope).double()
+        codes, e = _quantise(z, fmt)
+        if mode == 'keep_sign':
+            codes = _kept(z, codes, e, sc, sh, fmt)
+        assert torch.equal(ck.codes[0, c, :LONG].double()[None], codes) and torch.equal(ck.scales[0, c, :nb].int() - 127, e[0].int()), c
+        v = _values(codes, e)[0]
+        a = (v * sc + sh).float()
+        a = torch.where(a > 0, a, a * slope).double()
+        assert torch.equal(backs[0][0, c], v.to(dtype))
+        # the activation is rounded as it is formed (a second time where it is negative, by the slope) and to its type
+        assert bool(((backs[1][0, c].double() - a).abs() <= (HALF[dtype] + 2 * U) * a.abs() + 2.0 ** -140).all()), c
+
+
+@pytest.mark.parametrize('K,use2', [(0, False), (2, False), (3, True)])
+@pytest.mark.parametrize('fmt', ['int8', 'e4m3'])
+def test_backward_past_the_caches(fmt, K, use2):
+    """Rows of which the first ones are read past the caches, and the last ones not; tolerances as for short rows (test_gpu_act8)."""
+    from deepwmh_amd import act8
+    C = 40
+    g = torch.Generator(device='cuda').manual_seed(35)
+    x, _ = _long(C, g)
+    ck = act8.pack(x, fmt)
+    mean, rstd = x.double().mean(-1), 1 / (x.double().var(-1, unbiased=False) + 1e-5).sqrt()
+    gamma, beta = 1 + 0.2 * torch.randn(C, device='cuda', generator=g), 0.2 * torch.randn(C, device='cuda', generator=g)
+    mr = torch.stack([mean, rstd], -1).float()
+    ss = torch.stack([gamma * rstd, beta - mean * gamma * rstd], -1).float()
+    new = lambda *s: 1e-2 * torch.randn(s, device='cuda', generator=g)           # noqa: E731
+    g1, g2, dl, wseg = new(1, C, LONG), new(1, C, LONG) if use2 else None, new(1, K, LONG) if K else None, new(K, C) if K else None
+    assert C * LONG * (9 if use2 else 5) > 256 << 20
+    got = act8.instnorm_lrelu_backward(ck, ss, mr, gamma, g1=g1, g2=g2, dlogits=dl, wseg=wseg, slope=SLOPE)
+    y32 = act8.unpack(ck)
+    slope = float(np.float32(SLOPE))
+    for c in range(C):
+        y, sc, sh = y32[0, c].double(), ss[0, c, 0].double(), ss[0, c, 1].double()
+        z = y * sc + sh
+        terms = [t[0, c].double() for t in (g1, g2) if t is not None] + [wseg[k, c].double() * dl[0, k].double() for k in range(K)]
+        d = torch.where(z > 0, 1.0, slope)
+        dz, mag = sum(terms) * d, sum(t.abs() for t in terms) * d
+        xh = (y - mr[0, c, 0].double()) * mr[0, c, 1].double()
+        gr = gamma[c].double() * mr[0, c, 1].double()
+        dy = gr * (dz - dz.mean() - xh * (dz * xh).mean())
+        tol = 16 * U * gr.abs() * (mag + mag.mean() + xh.abs() * (mag * xh.abs()).mean()) + 2.0 ** -140
+        assert bool(((got.dy[0, c].double() - dy).abs() <= tol).all()), c
+        pairs = [(got.dbeta[c], dz.sum(), mag.sum()), (got.dgamma[c], (dz * xh).sum(), (mag * xh.abs()).sum()), (got.dbias[c], dy.sum(), tol.sum() / (16 * U))]
+        for k in range(K):
+            t = dl[0, k].double()
+            pairs.append((got.dwseg[k, c], (z * d * t).sum(), (t.abs() * ((z * d).abs() + sh.abs() + (y * sc).abs())).sum()))
+        for have, want, size in pairs:
+            assert abs(float(have) - float(want)) <= 16 * U * float(size) + 2.0 ** -140, c
