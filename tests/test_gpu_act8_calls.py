@@ -1,10 +1,13 @@
 """GPU tests of calls of the 8-bit checkpoint operators at the edges of what they accept: sizes of a real training step, infinite gradients, scales at
 both ends of the range, batches of many small products."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 import test_gpu_act8 as base
+import test_gpu_act8_trainer as steps
 from oracle import act8 as oa
 
 pytestmark = pytest.mark.gpu
@@ -227,3 +230,28 @@ def test_backward_past_the_caches(fmt, K, use2):
             pairs.append((got.dwseg[k, c], (z * d * t).sum(), (t.abs() * ((z * d).abs() + sh.abs() + (y * sc).abs())).sum()))
         for have, want, size in pairs:
             assert abs(float(have) - float(want)) <= 16 * U * float(size) + 2.0 ** -140, c
+
+
+# ---- a training step -----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('kind', ['tiny', 'aniso', 'wide'])
+@pytest.mark.parametrize('fmt,most', [('int8', 0.05), ('e4m3', 0.13)])
+def test_every_gradient_of_a_checkpointed_step_is_finite(kind, fmt, most, tiny_net):
+    """And near the exact one (bounds of test_gpu_act8_trainer).  Only a gradient that is identically zero has no relative error: a head whose weight in
+    the loss is zero, where the checkpointed one is zero too."""
+    from deepwmh_amd.trainer import UNetTrainer
+    plan, sd, x, lab = steps._setup(kind, tiny_net)
+    td = steps._targets(plan, lab)
+    plain, tr = UNetTrainer(plan, sd, 'cuda:0'), UNetTrainer(plan, sd, 'cuda:0', checkpoint8=fmt)
+    for t in (plain, tr):
+        t.forward(x)
+        t.backward(td)
+    a, b = steps._grads(plain), steps._grads(tr)
+    measured = 0
+    for n in a:
+        assert np.isfinite(a[n]).all() and np.isfinite(b[n]).all(), n
+        if not a[n].any():
+            assert not b[n].any(), n
+        elif kind == 'wide' and (n.endswith('conv.weight') or 'tu' in n or 'seg' in n):
+            measured += 1
+            assert math.isfinite(np.linalg.norm(b[n])) and np.linalg.norm(a[n] - b[n]) <= most * np.linalg.norm(a[n]), n
+    assert measured > 10 or kind != 'wide'
