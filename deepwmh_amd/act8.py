@@ -8,8 +8,9 @@ nearest even.  A block that holds an infinity or a NaN reads NaN as a whole.
   pack / unpack                        a tensor to its checkpoint and back, optionally behind InstanceNorm + LeakyReLU
   pack_columns                         blocks along the other axis of a matrix: the operand of a product's gradient
   instnorm_lrelu_backward              backward pass of InstanceNorm + LeakyReLU (+ segmentation head) on a checkpoint of its input
-  product                              a b^T of two e4m3 checkpoints on the scaled 8-bit matrix instruction
-  convtranspose_weight_gradient        that product as the weight gradient of a transposed convolution (kernel = stride)
+  product                              a b^T of two e4m3 checkpoints: float32 results from the codes widened to bfloat16 (exact operands, float32
+                                       sums), bfloat16 results from the scaled 8-bit matrix instruction
+  convtranspose_weight_gradient        the float32 product as the weight gradient of a transposed convolution (kernel = stride)
 
 Calls are asynchronous on torch's current stream of the tensors' device; outputs and workspaces come from torch's allocator unless given.
 There is no CPU path, and nothing is recorded for autograd: a tensor that requires grad is refused while grad mode is on.
@@ -204,7 +205,7 @@ def instnorm_lrelu_backward(ck, ss, mean_rstd, gamma=None, g1=None, g2=None, dlo
     """Backward pass of a = lrelu(instnorm(y)) on the checkpoint of y: ss and mean_rstd [N, C, 2] of the forward pass, gamma [C]; the gradient of
     a is g1 + g2 + wseg^T dlogits (any of the three; g1, g2 of y's shape, dlogits [N, K, ...], wseg [K, C]).  Returns InstNormGrads: dy of y's
     shape, dgamma, dbeta, dbias (the sum of dy) [C], and dwseg [K, C] or None.  `out`: an InstNormGrads of tensors to write into; one that is
-    None there is not formed (dy always is; it may be g1 or g2 itself)."""
+    None there is not formed (dy always is; it may be g1 or g2 itself).  N C is at most 65535 and K 4."""
     what = 'instnorm_lrelu_backward'
     N, Cc = ck.shape[:2]
     if min(N, Cc, ck.length) < 1:
@@ -251,8 +252,10 @@ def instnorm_lrelu_backward(ck, ss, mean_rstd, gamma=None, g1=None, g2=None, dlo
 
 def product(a, b, dtype=torch.float32, sum_batches=False, out=None):
     """a [B, M, K] and b [B, N, K] packed to e4m3 -> a b^T: [B, M, N], or [M, N] summed over the batch.  A float32 result is a
-    sum in float32; a bfloat16 result comes from the 8-bit matrix instruction, twice as fast, whose sums of eight neighbours keep 14 bits of the
-    largest product (1.5e-5 of a sum of random terms, against the result's rounding of 2^-8).  Its gradients are products again, of operands packed along the other axis (pack_columns):
+    sum in float32 of codes widened exactly to bfloat16 (a value below 2^-126 may lose bits); a bfloat16 result comes from the scaled 8-bit matrix
+    instruction, twice as fast, whose sums of eight neighbours keep 14 bits of the largest product: 1.5e-5 of a sum of random terms, against the
+    result's rounding of 2^-8, and at most 2^-10 of the sum of |terms|, which is more than that rounding where terms cancel.  A product's gradients
+    are products again, of operands packed along the other axis (pack_columns):
     da = product(pack(dc), pack_columns(b)), db = product(pack_columns(dc), pack_columns(a))."""
     if a.codes.dtype != torch.float8_e4m3fn or b.codes.dtype != torch.float8_e4m3fn:
         raise TypeError('product: e4m3 operands expected, got %s and %s' % (a.fmt, b.fmt))
@@ -279,7 +282,8 @@ def product(a, b, dtype=torch.float32, sum_batches=False, out=None):
 def convtranspose_weight_gradient(x, ss, dy, slope=LRELU_SLOPE, out=None):
     """Weight gradient [Cin, Cout, kt, 2, 2] of a transposed convolution with kernel = stride = (kt, 2, 2), kt 1 or 2, from its float32 input
     x [N, Cin, D, H, W] (behind InstanceNorm + LeakyReLU where ss [N, Cin, 2] is given) and dy [N, Cout, kt D, 2 H, 2 W]: both are packed to
-    e4m3 in blocks of 128 low-resolution voxels and multiplied on the 8-bit matrix instruction."""
+    e4m3 in blocks of 128 low-resolution voxels, and the codes multiplied as in `product` with a float32 result: widened exactly to bfloat16 with
+    their scale, sums in float32."""
     what = 'convtranspose_weight_gradient'
     if x.dim() != 5 or dy.dim() != 5 or x.shape[0] != dy.shape[0]:
         raise ValueError('%s: [N, C, D, H, W] expected, got %s and %s' % (what, tuple(x.shape), tuple(dy.shape)))

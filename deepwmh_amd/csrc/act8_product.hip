@@ -293,7 +293,9 @@ __global__ __launch_bounds__(64 * WM * WN, (MT * NT == 8 ? 2 : 1)) void act8_pro
 //    of 64 bytes a row, which ask for every line twice (455).
 //  * All loads are LDS-DMA, the scales' dwords too (the block's own, with every block), and return in order, so that s_waitcnt counts them.  Past the end
 //    the last block is fetched again, so that the counts hold.
-// 8192^3 410 us = 2680 TFLOP/s (the eight waves above with their two buffers 450); without its memory traffic the loop takes 343, the traffic alone 277.
+// 8192^3 402 to 410 us = 2700 TFLOP/s in a steady run (the eight waves above with their two buffers 450; the library's product of the same codes without
+// block scales 329 to 340); without its memory traffic the loop takes 343, the traffic alone 277.  The clock moves under this load: of 60 launches in a row
+// the tenth took 540 us and the last 406, and between other kernels 450 to 500 are usual.
 __global__ __launch_bounds__(256, 1) void act8_product_deep_kernel(const Act8Prod p) {
     constexpr int UNIT = 64 * ACT8_BLOCK, NS = 19, SCALES = NS * UNIT;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];    // NS units, then two sets of 512 scale dwords
@@ -452,7 +454,8 @@ static void launch_join(bool wide, const float* slabs, void* c, size_t n, int P,
     else hipLaunchKernelGGL(act8_product_join_kernel<false>, dim3(blocks), dim3(256), 0, st, slabs, c, n, P);
 }
 
-// Tiles and parts, by measurement (us, float32 / bfloat16 result, replayed graphs of ten calls):
+// Tiles and parts, by measurement (us, float32 / bfloat16 result, replayed graphs of ten calls) of one to three items.  Tiles of many small items are counted
+// like those of one large matrix, whether or not they are full: 256 x (64 x 64 x 512) takes 18 / 11 us on 256 tiles of 256 x 256.
 //  0  256 x 256, one workgroup a CU: from 192 tiles on (4096^3: 109 / 58, tile 1 136 / 80; with 128 tiles, 4096 x 2048 x 1024, 30 / 22 against
 //     24 / 16 of tile 1).  bfloat16 results of sums from 4096 k on by four waves (8192 x 8192 x 16384 845, by eight 908; 4096^3 58 / 62; 3600 x 3900 x
 //     3500 52 / 51, 3600 x 3900 x 2100 38 / 35: a longer start and end), the others by eight of 128 x 64.

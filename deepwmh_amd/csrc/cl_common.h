@@ -41,16 +41,16 @@ __device__ __forceinline__ float cl_ld_uniform(const float* p) {
 
 // One 16-byte piece = 8 consecutive channels of one voxel: lrelu(x * scale + shift), back to bf16.
 // sc / sh: the 8 channels' scale and shift; slope 1 with scale 1 / shift 0 = identity (a source without pending norm).
-// UNPACKED: plain v_fma_f32 / v_mul_f32 / v_max_f32 (conv3d_common.h::wmh_norm_lrelu) -- for a staging wave that shares its SIMD with a
-// consumer wave's MFMA stream: packed fp32 instructions do not overlap with it (cl_conv3_kernel's stride-1 layers 3-8 % faster,
-// round 3).  The one-role kernels (stride 2, first layer, transposed convolution), where the same wave issues the MFMAs afterwards,
-// keep the packed form: half the instructions (measured: 0.69 against 0.71 ms on the first strided layer).  Same roundings either way.
-template <bool UNPACKED = false>
+// FIXED: the instructions as written (conv3d_common.h::wmh_norm_lrelu) -- for a staging wave that shares its SIMD with a consumer wave's
+// MFMA stream.  The one-role kernels (stride 2, transposed convolution), where the same wave issues the MFMAs afterwards, leave their order
+// to the compiler (first strided layer of 16 patches 1.00 ms, 1.21 with FIXED).  The build forbids packed fp32 instructions in either.  Same
+// roundings.
+template <bool FIXED = false>
 __device__ __forceinline__ cl_u32x4 cl_transform8(const cl_u32x4 u, const float (&sc)[8], const float (&sh)[8], float slope) {
     cl_u32x4 w;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        if constexpr (UNPACKED) {
+        if constexpr (FIXED) {
             const float x0 = __builtin_bit_cast(float, u[p] << 16), x1 = __builtin_bit_cast(float, u[p] & 0xFFFF0000u);
             w[p] = cl_pack2(wmh_norm_lrelu(x0, sc[2 * p], sh[2 * p], slope), wmh_norm_lrelu(x1, sc[2 * p + 1], sh[2 * p + 1], slope));
         } else {

@@ -562,12 +562,13 @@ int wmh_act8_in_lrelu_bwd(const uint8_t* codes, const uint8_t* scales, int fmt, 
                           float slope, void* stream);
 /* c[b] = a[b] b[b]^T, or with sum != 0 one c for the whole batch: a [B][M][K], b [B][N][K] packed e4m3, c [M][N] row-major per item,
  * dtype WMH_F32 or WMH_BF16; K = 0 gives zeros.  WMH_F32: sums of float32 (1e-7); WMH_BF16: on the 8-bit matrix instruction, whose
- * sums of eight neighbours keep 14 bits of the largest product (1.5e-5 of a sum of random terms), at twice the rate.  workspace: 16-byte aligned (may be NULL where the size is 0). */
+ * sums of eight neighbours keep 14 bits of the largest product (1.5e-5 of a sum of random terms, at most 2^-10 of the sum of |terms|), at
+ * twice the rate.  workspace: 16-byte aligned (may be NULL where the size is 0). */
 size_t wmh_act8_product_workspace_floats(int B, int M, int N, size_t K, int sum);
 int wmh_act8_product(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, void* c, int dtype,
                      float* workspace, int B, int M, int N, size_t K, int sum, void* stream);
 /* wmh_convtranspose3d_wgrad with both operands of the product packed to e4m3 in blocks of 128 low-resolution voxels (x behind its
- * InstanceNorm + LeakyReLU): dW [Cin][Cout][kt][2][2].  workspace: 16-byte aligned. */
+ * InstanceNorm + LeakyReLU) and multiplied as for a WMH_F32 result: dW [Cin][Cout][kt][2][2].  workspace: 16-byte aligned. */
 size_t wmh_act8_convtranspose3d_wgrad_workspace_bytes(int N, int Cin, int Cout, int D, int H, int W, int kt);
 int wmh_act8_convtranspose3d_wgrad(const float* x, const float* ss, const float* dY, float* dW, void* workspace, int N, int Cin,
                                    int Cout, int D, int H, int W, int kt, float slope, void* stream);
