@@ -69,6 +69,8 @@ class Act8:
         if fmt not in FORMATS:
             raise ValueError('format must be int8 or e4m3, got %r' % (fmt,))
         shape = tuple(shape)
+        if len(shape) < 3 or min(shape) < 0:
+            raise ValueError('Act8: shape [N, C, ...] expected, got %s' % (shape,))
         length = _length(shape)
         pitch, spitch = _pitches(length)
         self = cls.__new__(cls)                                 # (parts made to fit need no checks)
@@ -225,7 +227,7 @@ def instnorm_lrelu_backward(ck, ss, mean_rstd, gamma=None, g1=None, g2=None, dlo
         if not 1 <= K <= 4 or wseg is None:
             raise ValueError('%s: dlogits needs wseg and 1 to 4 classes, got %s' % (what, tuple(dlogits.shape)))
         _f32(what, 'dlogits', dlogits, (N, K) + ck.shape[2:])
-        if wseg.dtype != torch.float32 or wseg.numel() != K * Cc or wseg.shape[0] != K or not wseg.is_contiguous():
+        if wseg.dtype != torch.float32 or wseg.numel() != K * Cc or wseg.shape[:1] != (K,) or not wseg.is_contiguous():
             raise ValueError('%s: wseg must be contiguous float32 %s, got %s %s' % (what, (K, Cc), wseg.dtype, tuple(wseg.shape)))
     dev = _device(what, ck, ss, mean_rstd, gamma, g1, g2, dlogits, wseg)
     lib = _lib.load()

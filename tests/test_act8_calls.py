@@ -29,3 +29,12 @@ def test_a_tensor_that_requires_grad_is_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match='no CPU path'):
             call()
             pytest.fail('call %d was taken' % k)
+
+
+def test_shapes_that_are_no_checkpoints_are_refused():
+    for shape in ((2, 3), (1, 2, -5), ()):
+        with pytest.raises(ValueError, match='expected'):
+            act8.Act8.empty(shape, 'int8', 'cpu')
+    st = torch.zeros(1, 1, 2)
+    with pytest.raises(ValueError, match='wseg'):               # (a number is no [K, C])
+        act8.instnorm_lrelu_backward(_ck((1, 1, 5)), st, st, dlogits=torch.zeros(1, 1, 5), wseg=torch.tensor(1.0))
